@@ -124,6 +124,20 @@ __device__ __forceinline__ unsigned decode_bf16(unsigned pair, float scale) {
     return *reinterpret_cast<const unsigned*>(&p);
 }
 
+// The sum of a row of gy over some steps, by a warp.
+template <typename T>
+__device__ __forceinline__ float row_sum(const WgradArgs& P, int o, long long first, int steps, int positions, int lane) {
+    float s = 0.0f;
+    for (long long step = first; step < first + steps; ++step) {
+        const long long sample = step / P.steps_n, p = (step - sample * P.steps_n) * positions, left = min((long long)positions, P.n - p);
+        const T* g = reinterpret_cast<const T*>(P.gy) + (sample * P.co + o) * P.n + p;
+        for (int i = lane; i < left; i += 32) s += ndc::to_f32(g[i]);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    return s;
+}
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ WgradArgs P, int stages) {
     typedef Step<T, VEC> S;
@@ -240,6 +254,13 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
                 float ones = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) ones += k == P.ct ? v[i] : v[16 + i];
+                // An infinity times the other rows' zeros is NaN, whatever the sum is: it is made again, without them
+                unsigned odd = __ballot_sync(0xffffffffu, o < P.co && ok && !(fabsf(ones) < __uint_as_float(kInfinite)));
+                for (; odd; odd &= odd - 1) {
+                    const int l = __ffs(odd) - 1;
+                    const float sum = row_sum<T>(P, o0 + 32 * quarter + l, first, steps, S::POSITIONS, lane);
+                    if (lane == l) ones = sum;
+                }
                 if (o < P.co && ok) out[(long long)P.ci * P.co] = ones;
             }
         }
