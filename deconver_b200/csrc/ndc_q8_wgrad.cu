@@ -98,7 +98,7 @@ template <bool VEC> struct Octet<float, VEC> {
             for (int i = 0; i < 8; ++i) v[i] = i < left ? __ldg(p + i) : 0.0f;
         }
     }
-    // the leading eight bits of each value, the next eight, and the last; an infinity has no remainder
+    // the leading eight bits of each value, the next eight, and the last; an infinity has no remainder (a NaN does: it may have its bits below the leading ones)
     __device__ __forceinline__ void store(unsigned char* to) {
 #pragma unroll
         for (int t = 0; t < 3; ++t) {
@@ -109,8 +109,8 @@ template <bool VEC> struct Octet<float, VEC> {
                 w[i / 2] = __byte_perm(a, b, 0x7632);
                 if (t < 2) {
                     const unsigned ha = a & 0xffff0000u, hb = b & 0xffff0000u;
-                    v[i] = (ha & 0x7fffffffu) == kInfinite ? 0.0f : v[i] - __uint_as_float(ha);
-                    v[i + 1] = (hb & 0x7fffffffu) == kInfinite ? 0.0f : v[i + 1] - __uint_as_float(hb);
+                    v[i] = (a & 0x7fffffffu) == kInfinite ? 0.0f : v[i] - __uint_as_float(ha);
+                    v[i + 1] = (b & 0x7fffffffu) == kInfinite ? 0.0f : v[i + 1] - __uint_as_float(hb);
                 }
             }
             *reinterpret_cast<uint4*>(to + t * MT * kRowBytes) = make_uint4(w[0], w[1], w[2], w[3]);
