@@ -742,8 +742,11 @@ void held_project(const Tensor& x, int64_t batch, int64_t ci, int64_t co, int64_
 // held operand ndc_q8_wgrad decodes once for each 128 outputs.  Microseconds, ndc_q8_wgrad and the other way, at batch x (inputs ->
 // outputs) x positions: 16 x (512 -> 2048) x 4096 298 and 224, 16 x (256 -> 1024) x 16384 283 and 256, 4 x (2048 -> 2048) x 8192
 // 575 and 264; but 16 x (256 -> 1024) x 4096 89 and 110, 8 x (1024 -> 1024) x 1000 60 and 79, 2 x (64 -> 256) x 262144 66 and 150.
-bool library_wgrad(const Tensor& g, int64_t co, int64_t ci, int64_t rows) {
-    return g.scalar_type() == at::kBFloat16 && co * ci >= 1 << 18 && 2.0 * (double)rows * (double)(co * ci) >= 1e11;
+// (All of what is read back is in memory meanwhile, a bfloat16 copy of the input.)  Rows of whole vectors only: for others the library has its
+// convolution, whose sums need not come in the same order every time, and which is the slower one: 1 x (512 -> 512) x 200003 641 us for 1006,
+// 4 x (512 -> 512) x 100003 1266 for 4483, 16 x (512 -> 2048) x 4095 707 for 1098 (with the bias gradient).
+bool library_wgrad(const Tensor& g, int64_t co, int64_t ci, int64_t batch, int64_t n) {
+    return g.scalar_type() == at::kBFloat16 && n % 8 == 0 && co * ci >= 1 << 18 && 2.0 * (double)batch * (double)n * (double)(co * ci) >= 1e11;
 }
 
 // y = w x (+ bias); what the backward knows of x is held in 8 bits.  `products`: those of operands held in 8 bits, each in
@@ -799,7 +802,7 @@ struct HeldLinearNode : public torch::autograd::Function<HeldLinearNode> {
             c10::cuda::CUDAGuard guard(w.device());
             const Tensor g = like(grads[0], w);
             const Slabs s = slabs(g);
-            const int64_t ci = shape[1], co = w.size(0), rows = (int64_t)s.batch * s.n;
+            const int64_t ci = shape[1], co = w.size(0);
             if (ctx->needs_input_grad(0)) {
                 out[0] = at::empty(shape, g.options());
                 if (!s.n || !ci) out[0].zero_();
@@ -811,7 +814,7 @@ struct HeldLinearNode : public torch::autograd::Function<HeldLinearNode> {
                 else {
                     // the bias gradient from the same pass over g
                     const auto type = (at::ScalarType)d["type"].toInt();
-                    const bool library = !products && library_wgrad(g, co, ci, rows);
+                    const bool library = !products && library_wgrad(g, co, ci, s.batch, s.n);
                     out[1] = library ? weight_grad(g, read(held, shape, g.scalar_type()), w, s.batch, s.n) : at::empty(w.sizes(), w.options());
                     const bool bias = !library && d["bias"].toBool() && ctx->needs_input_grad(2) && (type == at::kFloat || type == at::kBFloat16);
                     const int code = type == at::kBFloat16 ? NDC_BF16 : NDC_F32;

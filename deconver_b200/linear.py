@@ -45,6 +45,7 @@ def channel_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
 
     checkpoint="fp8": the backward pass knows the input as it is held in 8 bits (`deconver_b200.fp8`), blocks along the
         positions: the weight's gradient is that of what is held; the result and the other gradients are not touched.
+        (Of large bfloat16 layers, 2^18 weights and 10^11 operations, it is read back whole for that gradient.)
     products="fp8": the products are of operands held in 8 bits, in blocks of 128 along what they are summed over:
         y (blocks of input channels), the input's gradient (of output channels), the weight's (of positions, from the
         checkpoint, so that the input is kept in 8 bits here too).  Sums are float32; the bias and its gradient are not
