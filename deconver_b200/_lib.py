@@ -24,12 +24,13 @@ SYMBOLS = (
     "ndc_fwd", "ndc_bwd_workspace_bytes", "ndc_bwd", "ndc_bwd_static", "ndc_gconv",
     "ndc_probe_fp32_fma", "ndc_inorm_workspace_bytes", "ndc_inorm_last_error", "ndc_inorm_fwd",
     "ndc_inorm_bwd", "ndc_bias_grad_workspace_bytes", "ndc_bias_last_error", "ndc_bias_add",
-    "ndc_bias_grad", "ndc_bias_gelu_fwd", "ndc_bias_gelu_bwd", "ndc_proj_wgrad_workspace_bytes",
+    "ndc_bias_grad", "ndc_bias_round", "ndc_bias_gelu_fwd", "ndc_bias_gelu_bwd", "ndc_proj_wgrad_workspace_bytes",
     "ndc_proj_last_error", "ndc_proj_wgrad", "ndc_proj_sum", "ndc_params_prepare", "ndc_params_grad",
     "ndc_wait_expired", "ndc_probe_wait", "ndc_row_pitch", "ndc_fwd_rows", "ndc_bwd_rows_workspace_bytes", "ndc_bwd_rows", "ndc_pad_rows", "ndc_unpad_rows",
     "ndc_q8_last_error", "ndc_q8_pitch", "ndc_q8_scales", "ndc_q8_hold", "ndc_q8_hold_sum", "ndc_q8_hold_channels", "ndc_q8_read", "ndc_q8_bias_gelu_fwd",
     "ndc_q8_bias_gelu_bwd", "ndc_q8_product_workspace_bytes", "ndc_q8_product", "ndc_q8_project",
     "ndc_q8_wgrad_workspace_bytes", "ndc_q8_wgrad", "ndc_q8_linear_fwd_applies", "ndc_q8_linear_fwd",
+    "ndc_q8_linear_fwd_parts_applies", "ndc_q8_linear_fwd_parts",
 )
 
 
@@ -142,6 +143,8 @@ def load():
     lib.ndc_params_grad.restype = ctypes.c_int
     lib.ndc_params_grad.argtypes = [ctypes.c_int32, vp, fp, ctypes.c_int64, vp, fp, ctypes.c_int64, vp, vp]
     i64 = ctypes.c_int64
+    lib.ndc_bias_round.restype = ctypes.c_int
+    lib.ndc_bias_round.argtypes = [i32, i32, i64, vp, vp, vp, i64, vp]
     lib.ndc_q8_last_error.restype = ctypes.c_char_p
     for name in ("ndc_q8_pitch", "ndc_q8_scales"):
         getattr(lib, name).restype = i64
@@ -168,10 +171,11 @@ def load():
     lib.ndc_q8_wgrad_workspace_bytes.argtypes = [i32, i32, i32, i64, i32]
     lib.ndc_q8_wgrad.restype = ctypes.c_int
     lib.ndc_q8_wgrad.argtypes = [i32, i32, i32, i64, i32, vp, vp, vp, vp, vp, i32, vp, ctypes.c_size_t, vp]
-    lib.ndc_q8_linear_fwd_applies.restype = i32
-    lib.ndc_q8_linear_fwd_applies.argtypes = [i32, i32, i32, i64]
-    lib.ndc_q8_linear_fwd.restype = ctypes.c_int
-    lib.ndc_q8_linear_fwd.argtypes = [i32, i32, i32, i64, vp, vp, vp, i32, vp, vp, vp, vp]
+    for name in ("ndc_q8_linear_fwd", "ndc_q8_linear_fwd_parts"):
+        getattr(lib, name + "_applies").restype = i32
+        getattr(lib, name + "_applies").argtypes = [i32, i32, i32, i64]
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [i32, i32, i32, i64, vp, vp, vp, i32, vp, vp, vp, vp]
     _lib = lib
     return lib
 

@@ -55,6 +55,29 @@ __global__ void __launch_bounds__(kNT) bias_add_kernel(T* __restrict__ y, long l
     }
 }
 
+// y = v + bias rounded once: v of whole rows of `count` values, y's rows `pitch` apart.
+template <bool VEC>
+__global__ void __launch_bounds__(kNT) bias_round_kernel(const float* __restrict__ v, __nv_bfloat16* __restrict__ y, long long count, long long pitch,
+                                                         int channels, int nsplit, const float* __restrict__ bias) {
+    typedef Vec16<__nv_bfloat16> V;
+    const long long slab = blockIdx.x / nsplit;
+    const int part = blockIdx.x % nsplit;
+    const float* vs = v + slab * count;
+    __nv_bfloat16* ys = y + slab * pitch;
+    const float b = bias[slab % channels];
+    long long begin, end;
+    part_range(count, nsplit, part, V::N, begin, end);
+    if (VEC) {
+        for (long long i = begin + (long long)threadIdx.x * V::N; i < end; i += (long long)kNT * V::N) {
+            const float4 lo = *reinterpret_cast<const float4*>(vs + i), hi = *reinterpret_cast<const float4*>(vs + i + 4);
+            const float f[8] = {lo.x + b, lo.y + b, lo.z + b, lo.w + b, hi.x + b, hi.y + b, hi.z + b, hi.w + b};
+            *reinterpret_cast<V::raw*>(ys + i) = V::pack(f);
+        }
+    } else {
+        for (long long i = begin + threadIdx.x; i < end; i += kNT) ys[i] = __float2bfloat16_rn(vs[i] + b);
+    }
+}
+
 // partial[slab * nsplit + part] = sum of the part
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kNT) bias_grad_partial_kernel(const T* __restrict__ gy, long long sp,
@@ -244,6 +267,26 @@ int ndc_bias_add(int32_t batch, int32_t channels, int64_t spatial, int32_t dtype
     ndc::launched();
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return bias_fail(NDC_ERR_CUDA, "bias add: %s", cudaGetErrorString(e));
+    return NDC_OK;
+}
+
+int ndc_bias_round(int32_t batch, int32_t channels, int64_t count, const float* v, const float* bias, void* y, int64_t pitch, void* stream) {
+    if (!v || !bias || !y) return bias_fail(NDC_ERR_INVALID, "bias round: v, bias and y must not be NULL");
+    const int st = check(batch, channels, count, NDC_BF16);
+    if (st != NDC_OK) return st;
+    if (pitch < count) return bias_fail(NDC_ERR_INVALID, "bias round: rows overlap");
+    if (((uintptr_t)v | (uintptr_t)bias) % 4 || (uintptr_t)y % 2) return bias_fail(NDC_ERR_ALIGNMENT, "bias round: a tensor does not lie on its elements' size");
+    const long long slabs = (long long)batch * channels;
+    const int nsplit = choose_split(slabs, count);
+    const bool vec = count % 8 == 0 && pitch % 8 == 0 && ((uintptr_t)v | (uintptr_t)y) % 16 == 0;
+    const unsigned grid = (unsigned)(slabs * nsplit);
+    cudaStream_t s = (cudaStream_t)stream;
+    typedef __nv_bfloat16 bf16;
+    if (vec) bias_round_kernel<true><<<grid, kNT, 0, s>>>(v, (bf16*)y, count, pitch, channels, nsplit, bias);
+    else bias_round_kernel<false><<<grid, kNT, 0, s>>>(v, (bf16*)y, count, pitch, channels, nsplit, bias);
+    ndc::launched();
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return bias_fail(NDC_ERR_CUDA, "bias round: %s", cudaGetErrorString(e));
     return NDC_OK;
 }
 

@@ -12,6 +12,10 @@
 // positions as rows it stored 2 bytes for every four instructions: 78 us at 2 x (64 -> 256) x 64^3).  Two groups of
 // four warps do that, of one accumulator while the next is being computed (up to 256 channels: two of them fit).  What bounds it:
 // the bytes of x, y and what is held, 370 MB in 66 us there (5.6 TB/s).
+//
+// A w that does not fit goes in parts of 128 to 512 outputs, CTAs each; those of a tile run at the same time, have x from the L2
+// cache, and hold a part of its blocks each.  2 x (64 -> 1024) x 64^3 252 us; 16 x (512 -> 2048) x 4096 236, bound by x's 1.1 GB out of the
+// L2 cache and 16 parts of nine CTAs.
 #include <algorithm>
 
 #include "ndc_b200.h"
@@ -43,7 +47,7 @@ struct ForwardArgs {
     unsigned char *values, *scales;          // or NULL
     long long n, pitch;
     int scale_pitch;
-    int ci, co, blocks, columns;             // blocks of input channels; co as the MMA takes it, a multiple of 128
+    int ci, co, blocks, columns;             // blocks of input channels; outputs of a part as the MMA takes them, a multiple of 128
     int tiles_n, tiles;                      // of a sample, of all
     int slots, buffers, staged;              // blocks of x in shared memory, accumulators, and places for results of a group
     unsigned* expired;
@@ -69,6 +73,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
     const int weights = P.blocks * P.columns * 128;                       // bytes
     const unsigned w_at = base + kHeader, y_at = w_at + weights, x_at = y_at + 2 * P.staged * kStaged;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int o0 = blockIdx.y * P.columns;                                // the part's first output
     if (threadIdx.x == 0) {
         for (int i = 0; i < P.slots; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1 + (P.values ? kHoldWarps : 0)); }
         for (int i = 0; i < 2; ++i) { mbar_init(dfull + 8 * i, 1); mbar_init(dempty + 8 * i, kStoreWarps); }
@@ -77,7 +82,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
     }
     if (threadIdx.x < 2) reinterpret_cast<volatile unsigned*>(smem + kGaveUp)[threadIdx.x] = 0u;
     if (warp == 0) tmem_alloc(slot_at, 512);
-    for (int j = threadIdx.x; j < (kHeader - kBias) / 4; j += kThreads) reinterpret_cast<float*>(smem + kBias)[j] = P.bias && j < P.co ? load_bias(P.bias, P.bias_bf16, j) : 0.0f;
+    for (int j = threadIdx.x; j < (kHeader - kBias) / 4; j += kThreads) reinterpret_cast<float*>(smem + kBias)[j] = P.bias && j < P.columns && o0 + j < P.co ? load_bias(P.bias, P.bias_bf16, o0 + j) : 0.0f;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -126,21 +131,30 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
                 }
                 fence_async_proxy();
                 group_sync(group);
-                if (copies) tma_store3(&map_y, p + (u & 1) * 64, u / 2 * MT, sample, y_at + (group * P.staged + place) * kStaged, p + (u & 1) * 64 < P.n);
+                const int o = o0 + u / 2 * MT;
+                if (copies) tma_store3(&map_y, p + (u & 1) * 64, o, sample, y_at + (group * P.staged + place) * kStaged, p + (u & 1) * 64 < P.n && o < P.co);
                 if (++place == P.staged) place = 0;
             }
         }
         if (copies) copies_done();
     } else if (warp < kStoreWarps + kHoldWarps) {
-        // sixteen lanes have a channel's 128 positions
+        // sixteen lanes have a channel's 128 positions; the parts take the blocks in turn
         const int w = warp - kStoreWarps, l = lane & 15, piece = l & 7;
         int slot = 0, phase = 0;
         for (int t = blockIdx.x; P.values && t < P.tiles && ok; t += gridDim.x) {
             const int sample = t / P.tiles_n, k = t - sample * P.tiles_n;
             const long long p = (long long)k * kBlock + 8 * l;
+            unsigned turn = (unsigned)t % gridDim.y * P.blocks % gridDim.y;        // the part that has the tile's first block
             for (int block = 0; block < P.blocks; ++block) {
                 ok = mbar_wait(full + 8 * slot, phase);
                 if (!ok) break;
+                const bool mine = turn == blockIdx.y;
+                if (++turn == gridDim.y) turn = 0;
+                if (!mine) {
+                    if (lane == 0) mbar_arrive(empty + 8 * slot);
+                    if (++slot == P.slots) { slot = 0; phase ^= 1; }
+                    continue;
+                }
                 const unsigned char* from = smem + (x_at - base) + slot * kBlockBytes + (l >> 3) * kHalf;
                 uint4 q[KC / (2 * kHoldWarps)];
 #pragma unroll
@@ -188,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
         if (lane == 0) {
             expect_bytes(wfull, weights);
             for (int block = 0; block < P.blocks; ++block)
-                for (int o = 0; o < P.columns; o += 16) tma_load(w_at + (block * P.columns + o) * 128, &map_w, block * KC, o, wfull);
+                for (int o = 0; o < P.columns; o += 16) tma_load(w_at + (block * P.columns + o) * 128, &map_w, block * KC, o0 + o, wfull);
             int issued = 0;
             for (int t = blockIdx.x; t < P.tiles && ok; t += gridDim.x) {
                 const int sample = t / P.tiles_n, p = (t - sample * P.tiles_n) * MT;
@@ -256,33 +270,45 @@ bool make_weight_map(CUtensorMap& map, const void* w, int co, int ci) {
 
 int weight_bytes(int ci, int co) { return (ci + KC - 1) / KC * ((co + MT - 1) / MT * MT) * 128; }
 
-}  // namespace
-}  // namespace q8
-}  // namespace ndc
+bool fits_positions(int batch, long long n) { return batch > 0 && n > 0 && n % 8 == 0 && n <= (1LL << 25) && (n + MT - 1) / MT <= (0x7fffffffLL - 1024) / batch; }
 
-using namespace ndc::q8;
-
-extern "C" {
-
-int32_t ndc_q8_linear_fwd_applies(int32_t batch, int32_t ci, int32_t co, int64_t n) {
-    return batch > 0 && ci > 0 && co > 0 && n > 0 && n % 8 == 0 && ci % 8 == 0 && co <= 512 && (long long)ci * co <= kMostWeights &&
-           weight_bytes(ci, co) <= kMostWeights && n <= (1LL << 25) && (n + MT - 1) / MT <= (0x7fffffffLL - 1024) / batch;
+// Parts of the outputs whose w fits shared memory, as wide as each other.
+struct Parts { int columns, parts; };
+Parts plan_parts(int ci, int co) {
+    const int most = std::min(512, kMostWeights / (128 * ((ci + KC - 1) / KC)) / MT * MT);
+    const int parts = (co + most - 1) / most;
+    return {((co + parts - 1) / parts + MT - 1) / MT * MT, parts};
 }
 
-int ndc_q8_linear_fwd(int32_t batch, int32_t ci, int32_t co, int64_t n, const void* x, const void* w, const void* bias, int32_t bias_dtype, void* y, void* values,
-                      void* scales, void* stream) {
+// CTAs of a part: those of the least rounds of CTAs times tiles.
+int ctas_of(int tiles, int parts) {
+    const long long sms = ndc::num_sms();
+    long long best = 1, best_time = 1LL << 62;
+    for (long long ctas : {sms / parts, (sms + parts - 1) / parts}) {
+        ctas = std::max(1LL, std::min(ctas, (long long)tiles));
+        const long long time = (ctas * parts + sms - 1) / sms * ((tiles + ctas - 1) / ctas);
+        if (time < best_time) { best_time = time; best = ctas; }
+    }
+    return (int)best;
+}
+
+int check_forward(const void* x, const void* w, const void* bias, int32_t bias_dtype, const void* y, const void* values, const void* scales) {
     if (!x || !w || !y || !values != !scales) return fail(NDC_ERR_INVALID, "q8 linear: x, w and y must not be NULL, values and scales come together");
     if (bias && bias_dtype != NDC_F32 && bias_dtype != NDC_BF16) return fail(NDC_ERR_INVALID, "q8 linear: bias dtype must be NDC_F32 or NDC_BF16");
-    if (!ndc_q8_linear_fwd_applies(batch, ci, co, n)) return fail(NDC_ERR_UNSUPPORTED, "q8 linear: not for %d x %d channels and these positions", ci, co);
+    return NDC_OK;
+}
+
+int launch_forward(int batch, int ci, int co, long long n, Parts parts, const void* x, const void* w, const void* bias, int32_t bias_dtype, void* y, void* values,
+                   void* scales, void* stream) {
     if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)values) & 15) return fail(NDC_ERR_ALIGNMENT, "q8 linear: x, w, y and values must lie on 16 bytes");
     if (off_elements(bias_dtype, {bias})) return fail(NDC_ERR_ALIGNMENT, "q8 linear: bias misaligned");
     if (ndc::tc::take_expired()) return fail(NDC_ERR_TIMEOUT, "a wait inside a kernel of an earlier call ran out after one second");
     ForwardArgs P{};
     P.bias = bias; P.bias_bf16 = bias_dtype == NDC_BF16; P.values = (unsigned char*)values; P.scales = (unsigned char*)scales;
     P.n = n; P.pitch = pitch_of(n); P.scale_pitch = (int)scales_of(n);
-    P.ci = ci; P.co = co; P.blocks = (ci + KC - 1) / KC; P.columns = (co + MT - 1) / MT * MT;
+    P.ci = ci; P.co = co; P.blocks = (ci + KC - 1) / KC; P.columns = parts.columns;
     P.tiles_n = (int)((n + MT - 1) / MT); P.tiles = P.tiles_n * batch;
-    const int weights = weight_bytes(ci, co);
+    const int weights = P.blocks * P.columns * 128;
     P.staged = kRoom - weights - 4 * kStaged >= 4 * kBlockBytes ? 2 : 1;
     P.slots = std::min(kMostSlots, (kRoom - weights - 2 * P.staged * kStaged) / kBlockBytes);
     P.buffers = P.columns <= 256 ? 2 : 1;
@@ -292,12 +318,44 @@ int ndc_q8_linear_fwd(int32_t batch, int32_t ci, int32_t co, int64_t n, const vo
     if (!make_tensor_map(map_x, x, 2, batch, ci, n, KC) || !make_tensor_map(map_y, y, 2, batch, co, n, MT) || !make_weight_map(map_w, w, co, ci)) return fail(NDC_ERR_CUDA, "q8 linear: the driver refused a tensor map");
     e = ndc::allow_smem(forward_kernel);
     if (e == cudaSuccess) {
-        forward_kernel<<<(unsigned)std::min(P.tiles, ndc::num_sms()), kThreads, 1024 + kHeader + weights + (size_t)2 * P.staged * kStaged + (size_t)P.slots * kBlockBytes,
-                         (cudaStream_t)stream>>>(map_x, map_w, map_y, P);
+        forward_kernel<<<dim3(ctas_of(P.tiles, parts.parts), parts.parts), kThreads,
+                         1024 + kHeader + weights + (size_t)2 * P.staged * kStaged + (size_t)P.slots * kBlockBytes, (cudaStream_t)stream>>>(map_x, map_w, map_y, P);
         ndc::launched();
         e = cudaGetLastError();
     }
     return e == cudaSuccess ? NDC_OK : fail(NDC_ERR_CUDA, "q8 linear: %s", cudaGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace q8
+}  // namespace ndc
+
+using namespace ndc::q8;
+
+extern "C" {
+
+int32_t ndc_q8_linear_fwd_applies(int32_t batch, int32_t ci, int32_t co, int64_t n) {
+    return ci > 0 && co > 0 && ci % 8 == 0 && co <= 512 && (long long)ci * co <= kMostWeights && weight_bytes(ci, co) <= kMostWeights && fits_positions(batch, n);
+}
+
+int ndc_q8_linear_fwd(int32_t batch, int32_t ci, int32_t co, int64_t n, const void* x, const void* w, const void* bias, int32_t bias_dtype, void* y, void* values,
+                      void* scales, void* stream) {
+    const int st = check_forward(x, w, bias, bias_dtype, y, values, scales);
+    if (st != NDC_OK) return st;
+    if (!ndc_q8_linear_fwd_applies(batch, ci, co, n)) return fail(NDC_ERR_UNSUPPORTED, "q8 linear: not for %d x %d channels and these positions", ci, co);
+    return launch_forward(batch, ci, co, n, Parts{(co + MT - 1) / MT * MT, 1}, x, w, bias, bias_dtype, y, values, scales, stream);
+}
+
+int32_t ndc_q8_linear_fwd_parts_applies(int32_t batch, int32_t ci, int32_t co, int64_t n) {
+    return ci > 0 && co > 0 && ci % 8 == 0 && ci <= 512 && co <= 1 << 20 && fits_positions(batch, n);
+}
+
+int ndc_q8_linear_fwd_parts(int32_t batch, int32_t ci, int32_t co, int64_t n, const void* x, const void* w, const void* bias, int32_t bias_dtype, void* y,
+                            void* values, void* scales, void* stream) {
+    const int st = check_forward(x, w, bias, bias_dtype, y, values, scales);
+    if (st != NDC_OK) return st;
+    if (!ndc_q8_linear_fwd_parts_applies(batch, ci, co, n)) return fail(NDC_ERR_UNSUPPORTED, "q8 linear: not for %d x %d channels and these positions", ci, co);
+    return launch_forward(batch, ci, co, n, plan_parts(ci, co), x, w, bias, bias_dtype, y, values, scales, stream);
 }
 
 }  // extern "C"

@@ -738,6 +738,35 @@ void held_project(const Tensor& x, int64_t batch, int64_t ci, int64_t co, int64_
                          stream()), ndc_q8_last_error());
 }
 
+// y = w x + bias of bfloat16 tensors, rounded once: the library's product in float32, and a pass that adds the bias, in parts of samples, or of
+// a sample's positions.  (Added to a y that is the bias, the library rounds its product first.)  16 x (2048 -> 512) x 4096 142 us, where the
+// exact layer, which rounds twice, takes 116; parts of 32 MiB or of all positions take 161 and 142.
+Tensor project_once(const Tensor& x, const Tensor& w, const Tensor& bias) {
+    constexpr int64_t kMost = 32 << 20;                        // values of a part
+    auto shape = x.sizes().vec();
+    shape[1] = w.size(0);
+    Tensor y = at::empty(shape, x.options());
+    const Slabs s = slabs(x);
+    const int64_t co = w.size(0), ci = s.channels;
+    const auto parts_of = [](int64_t count, int64_t most) { const int64_t parts = (count + most - 1) / most; return (count + parts - 1) / parts; };
+    const int64_t samples = parts_of(s.batch, std::max<int64_t>(1, kMost / (co * s.n)));
+    const int64_t positions = samples > 1 ? s.n : std::min(s.n, (parts_of(s.n, std::max<int64_t>(128, kMost / co)) + 127) / 128 * 128);
+    const Tensor b = as_f32(bias), v = at::empty({samples * co * positions}, x.options().dtype(at::kFloat));
+    cublasHandle_t handle = at::cuda::getCurrentCUDABlasHandle();
+    const float one = 1.0f, zero = 0.0f;
+    for (int64_t i = 0; i < s.batch; i += samples)
+        for (int64_t p = 0; p < s.n; p += positions) {
+            const int64_t count = std::min(samples, s.batch - i), n = std::min(positions, s.n - p);
+            const cublasStatus_t st = cublasGemmStridedBatchedEx(
+                handle, CUBLAS_OP_N, CUBLAS_OP_N, (int)n, (int)co, (int)ci, &one, static_cast<const at::BFloat16*>(ptr(x)) + i * ci * s.n + p, CUDA_R_16BF,
+                (int)s.n, (long long)(ci * s.n), ptr(w), CUDA_R_16BF, (int)ci, 0LL, &zero, ptr(v), CUDA_R_32F, (int)n, (long long)(co * n), (int)count,
+                CUBLAS_COMPUTE_32F, CUBLAS_GEMM_DEFAULT);
+            TORCH_CHECK(st == CUBLAS_STATUS_SUCCESS, "deconver_b200: projection GEMM failed (cuBLAS status ", (int)st, ")");
+            check(ndc_bias_round((int)count, (int)co, n, fptr(v), fptr(b), static_cast<at::BFloat16*>(ptr(y)) + i * co * s.n + p, s.n, stream()), ndc_bias_last_error());
+        }
+    return y;
+}
+
 // Where the weight gradient of a checkpoint is the library's product after all, of what is read back: large bfloat16 products, whose
 // held operand ndc_q8_wgrad decodes once for each 128 outputs.  Microseconds, ndc_q8_wgrad and the other way, at batch x (inputs ->
 // outputs) x positions: 16 x (512 -> 2048) x 4096 298 and 224, 16 x (256 -> 1024) x 16384 283 and 256, 4 x (2048 -> 2048) x 8192
@@ -758,18 +787,26 @@ struct HeldLinearNode : public torch::autograd::Function<HeldLinearNode> {
         shape[1] = w.size(0);
         const Slabs in = slabs(x);
         const int64_t co = w.size(0);
-        if (!products && in.n && co && x.scalar_type() == at::kBFloat16 && ndc_q8_linear_fwd_applies(in.batch, in.channels, (int)co, in.n) &&
-            ((uintptr_t)ptr(x) | (uintptr_t)ptr(w)) % 16 == 0) {
-            Tensor y = at::empty(shape, x.options());
-            if (held) *held = empty_held({in.batch, in.channels}, in.n, x);
-            const Tensor b = kernel_bias(bias);
-            check(ndc_q8_linear_fwd(in.batch, in.channels, (int)co, in.n, ptr(x), ptr(w), ptr(b), bias_code(b), ptr(y), held ? ptr(held->values) : nullptr,
-                                    held ? ptr(held->scales) : nullptr, stream()), ndc_q8_last_error());
-            return y;
+        // bfloat16 rows and weights of whole vectors: one pass that holds x.  Where w does not fit it whole, in parts if there is a bias, else the
+        // library's product, which is rounded once without one: with the pass that holds x 14, 32 and 136 us for 14, 41 and 236 at 2 x and 16 x
+        // (512 -> 2048) x 512 and 16 x (512 -> 2048) x 4096.  (With a bias 14, 41 and 236 for 26, 74 and 228 of the exact layer's launches.)
+        const bool whole = !products && in.n && co && x.scalar_type() == at::kBFloat16 && in.n % 8 == 0 && in.channels % 8 == 0;
+        if (whole && ((uintptr_t)ptr(x) | (uintptr_t)ptr(w)) % 16 == 0) {
+            const bool one = ndc_q8_linear_fwd_applies(in.batch, in.channels, (int)co, in.n);
+            if (one || (bias.defined() && ndc_q8_linear_fwd_parts_applies(in.batch, in.channels, (int)co, in.n))) {
+                Tensor y = at::empty(shape, x.options());
+                if (held) *held = empty_held({in.batch, in.channels}, in.n, x);
+                const Tensor b = kernel_bias(bias);
+                check((one ? ndc_q8_linear_fwd : ndc_q8_linear_fwd_parts)(in.batch, in.channels, (int)co, in.n, ptr(x), ptr(w), ptr(b), bias_code(b), ptr(y),
+                                                                           held ? ptr(held->values) : nullptr, held ? ptr(held->scales) : nullptr, stream()),
+                      ndc_q8_last_error());
+                return y;
+            }
         }
         if (!products || !in.n || !co) {
             if (held) *held = hold(x);
-            return LinearNode::run(x, w, bias);
+            // (ragged positions or channels: the exact layer's result, to the bit)
+            return whole && bias.defined() ? project_once(x, w, bias) : LinearNode::run(x, w, bias);
         }
         Tensor y = at::empty(shape, x.options());
         held_project(x, in.batch, in.channels, co, in.n, [&] { return hold(w.view({1, co, w.size(1)})); }, kernel_bias(bias), y, held);

@@ -266,6 +266,9 @@ int ndc_bias_add(int32_t batch, int32_t channels, int64_t spatial, int32_t dtype
                  const float *bias, void *stream);
 int ndc_bias_grad(int32_t batch, int32_t channels, int64_t spatial, int32_t dtype, const void *gy,
                   float *gbias, void *workspace, size_t workspace_bytes, void *stream);
+/* y[b, c, p] = v[b, c, p] + bias[c] as bfloat16, rounded once, for `count` positions; y's rows are `pitch` elements apart. */
+int ndc_bias_round(int32_t batch, int32_t channels, int64_t count, const float *v, const float *bias,
+                   void *y, int64_t pitch, void *stream);
 
 /*
  * The same bias fused with the erf-form GELU (`nn.GELU()`, approximate='none'; erf evaluated to
@@ -398,6 +401,11 @@ int32_t ndc_q8_linear_fwd_applies(int32_t batch, int32_t ci, int32_t co, int64_t
 int ndc_q8_linear_fwd(int32_t batch, int32_t ci, int32_t co, int64_t n, const void *x, const void *w,
                       const void *bias, int32_t bias_dtype, void *y, void *values, void *scales,
                       void *stream);
+/* The same for any number of outputs up to 2^20 of at most 512 inputs, in parts whose w fits (x from the L2 cache for each). */
+int32_t ndc_q8_linear_fwd_parts_applies(int32_t batch, int32_t ci, int32_t co, int64_t n);
+int ndc_q8_linear_fwd_parts(int32_t batch, int32_t ci, int32_t co, int64_t n, const void *x,
+                            const void *w, const void *bias, int32_t bias_dtype, void *y,
+                            void *values, void *scales, void *stream);
 
 /*
  * Measurement aid; no counterpart in the reference project.  Launches one kernel of

@@ -140,3 +140,35 @@ A = 4096       # an address that is aligned and never read
 def test_entry_points_refuse_bad_arguments(lib, status, call):
     assert call(lib) == status, lib.ndc_q8_last_error()
     assert lib.ndc_q8_last_error().startswith(b"q8 ")
+
+
+@pytest.mark.parametrize("status,call", [
+    (1, lambda l: l.ndc_q8_linear_fwd_parts(2, 8, 8, 8, A, None, None, 0, A, A, A, None)),
+    (1, lambda l: l.ndc_q8_linear_fwd_parts(2, 8, 8, 8, A, A, None, 0, A, None, A, None)),
+    (1, lambda l: l.ndc_q8_linear_fwd_parts(2, 8, 8, 8, A, A, A, 4, A, None, None, None)),
+    (2, lambda l: l.ndc_q8_linear_fwd_parts(2, 8, 8, 12, A, A, None, 0, A, None, None, None)),
+    (2, lambda l: l.ndc_q8_linear_fwd_parts(2, 12, 8, 8, A, A, None, 0, A, None, None, None)),
+    (2, lambda l: l.ndc_q8_linear_fwd_parts(2, 520, 8, 8, A, A, None, 0, A, None, None, None)),
+    (2, lambda l: l.ndc_q8_linear_fwd_parts(2, 512, 2 ** 20 + 1, 8, A, A, None, 0, A, None, None, None)),
+    (2, lambda l: l.ndc_q8_linear_fwd_parts(0, 8, 8, 8, A, A, None, 0, A, None, None, None)),
+    (2, lambda l: l.ndc_q8_linear_fwd_parts(2 ** 20, 8, 8, 2 ** 25, A, A, None, 0, A, None, None, None)),
+    (5, lambda l: l.ndc_q8_linear_fwd_parts(2, 512, 2048, 8, A, A + 8, None, 0, A, None, None, None)),
+    (5, lambda l: l.ndc_q8_linear_fwd_parts(2, 512, 2048, 8, A, A, None, 0, A + 2, None, None, None)),
+    (5, lambda l: l.ndc_q8_linear_fwd_parts(2, 512, 2048, 8, A, A, A + 2, 0, A, None, None, None)),
+])
+def test_the_forward_in_parts_refuses_bad_arguments(lib, status, call):
+    assert call(lib) == status, lib.ndc_q8_last_error()
+    assert lib.ndc_q8_last_error().startswith(b"q8 linear")
+
+
+@pytest.mark.parametrize("status,call", [
+    (1, lambda l: l.ndc_bias_round(2, 8, 8, A, None, A, 8, None)),
+    (1, lambda l: l.ndc_bias_round(2, 8, 0, A, A, A, 8, None)),
+    (1, lambda l: l.ndc_bias_round(2, 8, 8, A, A, A, 7, None)),
+    (2, lambda l: l.ndc_bias_round(2 ** 20, 2 ** 10, 8, A, A, A, 8, None)),
+    (5, lambda l: l.ndc_bias_round(2, 8, 8, A + 2, A, A, 8, None)),
+    (5, lambda l: l.ndc_bias_round(2, 8, 8, A, A, A + 1, 8, None)),
+])
+def test_the_rounded_bias_refuses_bad_arguments(lib, status, call):
+    assert call(lib) == status, lib.ndc_bias_last_error()
+    assert lib.ndc_bias_last_error().startswith(b"bias")
