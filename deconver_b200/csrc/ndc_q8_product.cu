@@ -41,7 +41,7 @@ struct ProductArgs {
     long long rows_a, rows_b;          // of the tensors
     int m, n, k;                       // of the product; k: of one sample
     int samples, kblocks;              // k runs over samples of kblocks blocks; sample s begins at row s * m of A, s * n of B
-    int slices;                        // of that sequence of blocks
+    int slices, slice0;                // of that sequence of blocks; the launch's first one
     const void* bias;                  // per column, float32 or bfloat16, or NULL
     int bias_bf16;
     void* out;                         // per slice m * n
@@ -76,7 +76,8 @@ __global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant
     const int n0 = blockIdx.x % tiles_n * NT, cols = min(NT, P.n - n0);
     const long long m0 = (long long)(blockIdx.x / tiles_n) * MT;
     const long long total = (long long)P.samples * P.kblocks;
-    const int first = (int)(total * blockIdx.z / P.slices), steps = (int)(total * (blockIdx.z + 1) / P.slices) - first;
+    const long long slice = P.slice0 + (int)blockIdx.z;
+    const int first = (int)(total * slice / P.slices), steps = (int)(total * (slice + 1) / P.slices) - first;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; ++s) { mbar_init(full + 8 * s, 3); mbar_init(empty + 8 * s, 1); }
@@ -191,17 +192,17 @@ __global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant
 // ---- host -------------------------------------------------------------------------------------
 
 template <int NT, typename T>
-cudaError_t launch(const CUtensorMap& a, const CUtensorMap& b, const ProductArgs& P, cudaStream_t st) {
+cudaError_t launch(const CUtensorMap& a, const CUtensorMap& b, const ProductArgs& P, int slices, cudaStream_t st) {
     auto kern = product_kernel<NT, T>;
     const cudaError_t e = ndc::allow_smem(kern);
     if (e != cudaSuccess) return e;
-    kern<<<dim3((unsigned)((P.m + MT - 1) / MT) * (unsigned)((P.n + NT - 1) / NT), 1, (unsigned)P.slices), kThreads, Shape<NT>::SMEM, st>>>(a, b, P);
+    kern<<<dim3((unsigned)((P.m + MT - 1) / MT) * (unsigned)((P.n + NT - 1) / NT), 1, (unsigned)slices), kThreads, Shape<NT>::SMEM, st>>>(a, b, P);
     ndc::launched();
     return cudaGetLastError();
 }
 
 // Columns of a tile: 256 halve what comes from the L2 cache for each row, if they leave a CTA for each multiprocessor.
-int columns_of(long long m, long long n, int slices) {
+int columns_of(long long m, long long n, long long slices) {
     if (n <= 64) return 64;
     const long long tiles = ((m + MT - 1) / MT) * ((n + 255) / 256) * slices;
     return n <= 128 || tiles < ndc::num_sms() ? 128 : 256;
@@ -213,14 +214,13 @@ int columns_of(long long m, long long n, int slices) {
 // and their sum) 4 slices take 75 us, 5 106, 7 88 and 9 73; the model says 73, 108, 84 and 71.  2048 x 512 of 1024 takes 7 us in
 // one slice, 11 in two.  For float32 results a slice has 32 blocks at most: the MMA cuts its sums off, and a chain of 128 shrinks
 // by about 128 2^-25.
-int plan_slices(int samples, long long m, long long n, long long k, int32_t dtype) {
-    const long long total = (long long)samples * ((k + KT - 1) / KT), limit = 65535;
-    const long long least = dtype == NDC_F32 ? std::min((total + 31) / 32, limit) : 1, most = std::max(least, std::min((total + 3) / 4, limit));
+Passes plan_slices(int samples, long long m, long long n, long long k, int32_t dtype) {
+    const long long total = (long long)samples * ((k + KT - 1) / KT), least = dtype == NDC_F32 ? (total + 31) / 32 : 1, most = std::max(least, (total + 3) / 4);
     long long best = least;
     double best_time = 1e300;
     auto consider = [&](long long slices) {
         slices = std::max(least, std::min(slices, most));
-        const int nt = columns_of(m, n, (int)slices), resident = nt == 256 ? 1 : 2;
+        const int nt = columns_of(m, n, slices), resident = nt == 256 ? 1 : 2;
         const long long ctas = ((m + MT - 1) / MT) * ((n + nt - 1) / nt) * slices, rounds = (ctas + resident * ndc::num_sms() - 1) / (resident * ndc::num_sms());
         const double step = nt == 256 ? 1.0 : nt == 128 ? 1.1 : 0.8, rest = nt == 256 ? 9.0 : 6.0;
         const double time = (double)rounds * ((double)((total + slices - 1) / slices) * step + rest) + (slices > 1 ? 6.0 + 2e-6 * (double)slices * (double)m * (double)n : 0.0);
@@ -232,7 +232,8 @@ int plan_slices(int samples, long long m, long long n, long long k, int32_t dtyp
             const int nt = n <= 64 ? 64 : width;
             consider((long long)rounds * (nt == 256 ? 1 : 2) * ndc::num_sms() / (((m + MT - 1) / MT) * ((n + nt - 1) / nt)));
         }
-    return (int)best;
+    const int nt = columns_of(m, n, best);
+    return plan_passes(best, (size_t)(m * n) * sizeof(float), ((m + MT - 1) / MT) * ((n + nt - 1) / nt));
 }
 
 }  // namespace
@@ -245,7 +246,7 @@ extern "C" {
 
 size_t ndc_q8_product_workspace_bytes(int32_t samples, int64_t m, int64_t n, int64_t k, int32_t dtype) {
     if (samples <= 0 || m <= 0 || n <= 0 || k <= 0) return 0;
-    return (size_t)plan_slices(samples, m, n, k, dtype) * m * n * sizeof(float);
+    return plan_slices(samples, m, n, k, dtype).places() * m * n * sizeof(float);
 }
 
 int ndc_q8_product(int32_t samples, int64_t m, int64_t n, int64_t k, int32_t dtype, const void* a_values, const void* a_scales,
@@ -266,8 +267,9 @@ int ndc_q8_product(int32_t samples, int64_t m, int64_t n, int64_t k, int32_t dty
         return fail(NDC_ERR_ALIGNMENT, "q8 product: out, bias or workspace misaligned");
     const bool split = samples > 1 || workspace;       // a sum over samples, or a long one, in slices
     if (split && (bias || rows != m)) return fail(NDC_ERR_INVALID, "q8 product: slices have neither bias nor groups of rows");
-    const int slices = split ? plan_slices(samples, m, n, k, dtype) : 1;
-    const size_t need = (size_t)slices * m * n * sizeof(float);
+    const Passes passes = split ? plan_slices(samples, m, n, k, dtype) : Passes{1, 1};
+    const int slices = passes.slices;
+    const size_t need = passes.places() * m * n * sizeof(float);
     if (split && (!workspace || workspace_bytes < need)) return fail(NDC_ERR_WORKSPACE, "q8 product: workspace of %zu bytes needed", need);
     if (ndc::tc::take_expired()) return fail(NDC_ERR_TIMEOUT, "a wait inside a kernel of an earlier call ran out after one second");
     ProductArgs P{};
@@ -276,23 +278,29 @@ int ndc_q8_product(int32_t samples, int64_t m, int64_t n, int64_t k, int32_t dty
     P.rows_a = (long long)samples * m; P.rows_b = (long long)samples * n;
     P.m = (int)m; P.n = (int)n; P.k = (int)k;
     P.samples = samples; P.kblocks = (int)kblocks; P.slices = slices;
-    P.bias = bias; P.bias_bf16 = bias_dtype == NDC_BF16; P.out = slices > 1 ? workspace : out; P.rows = rows;
+    P.bias = bias; P.bias_bf16 = bias_dtype == NDC_BF16; P.out = slices > 1 ? (float*)workspace + passes.first() * m * n : out; P.rows = rows;
     cudaError_t e = ndc::tc::expired_word(P.expired);
     if (e != cudaSuccess) return fail(NDC_ERR_CUDA, "q8 product: %s", cudaGetErrorString(e));
-    const int nt = columns_of(m, n, slices);
+    const int nt = columns_of(m, n, passes.each);
     CUtensorMap a, b;
     if (!make_map(a, a_values, P.rows_a, pitch_of(k), MT) || !make_map(b, b_values, P.rows_b, pitch_of(k), nt))
         return fail(NDC_ERR_CUDA, "q8 product: the driver refused a tensor map");
     cudaStream_t st = (cudaStream_t)stream;
     auto go = [&](auto type) {
         typedef decltype(type) T;
-        return nt == 64 ? launch<64, T>(a, b, P, st) : nt == 128 ? launch<128, T>(a, b, P, st) : launch<256, T>(a, b, P, st);
+        return nt == 64 ? launch<64, T>(a, b, P, passes.each, st) : nt == 128 ? launch<128, T>(a, b, P, passes.each, st) : launch<256, T>(a, b, P, passes.each, st);
     };
-    e = dtype == NDC_F32 || slices > 1 ? go(float()) : go(bf16());
-    if (e != cudaSuccess) return fail(NDC_ERR_CUDA, "q8 product: %s", cudaGetErrorString(e));
-    if (slices == 1) return NDC_OK;
-    return ndc_proj_sum(slices, m * n, dtype, (const float*)workspace, out, stream) == NDC_OK
-               ? NDC_OK : fail(NDC_ERR_CUDA, "q8 product: %s", ndc_proj_last_error());
+    for (int i = 0; i < passes.count(); ++i) {
+        P.slice0 = i * passes.each;
+        e = dtype == NDC_F32 || slices > 1 ? go(float()) : go(bf16());
+        if (e != cudaSuccess) return fail(NDC_ERR_CUDA, "q8 product: %s", cudaGetErrorString(e));
+        if (slices == 1) break;
+        const bool last = i + 1 == passes.count();
+        float* const places = (float*)workspace;
+        if (ndc_proj_sum(passes.added(i), m * n, last ? dtype : NDC_F32, places + passes.from(i) * m * n, last ? out : places + passes.to(i) * m * n, stream) != NDC_OK)
+            return fail(NDC_ERR_CUDA, "q8 product: %s", ndc_proj_last_error());
+    }
+    return NDC_OK;
 }
 
 }  // extern "C"

@@ -49,7 +49,7 @@ struct WgradArgs {
     int co, ci, ct, width;                    // inputs of a tile (a multiple of 16); ci, and one more with a bias
     int steps_n;                              // steps of a sample
     long long steps;                          // of all samples
-    int slices;
+    int slices, slice0;                       // of all; the launch's first one
     unsigned* expired;
 };
 
@@ -150,8 +150,8 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     const int o0 = blockIdx.x * MT, c0 = blockIdx.y * P.ct;
     const int inputs = min(P.ct, P.ci - c0), columns = columns_of(P.ct), bytes = S::bytes(columns);
-    const long long first = P.steps * blockIdx.z / P.slices;
-    const int steps = (int)(P.steps * (blockIdx.z + 1) / P.slices - first);
+    const long long slice = P.slice0 + (int)blockIdx.z, first = P.steps * slice / P.slices;
+    const int steps = (int)(P.steps * (slice + 1) / P.slices - first);
     constexpr int B = S::SUB * S::G;                      // where a stage's held rows begin
 
     if (tid == 0) {
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(256) wgrad_few_kernel(const float* __restrict_
     }
 }
 
-struct Plan { int ct, tiles_o, tiles_c, slices; long long steps; };
+struct Plan { int ct, tiles_o, tiles_c; long long steps; Passes passes; };
 
 // Inputs in equal tiles; slices for a CTA per multiprocessor, of at least 512 positions.
 Plan plan(int batch, int co, int ci, long long n, int positions, int32_t dtype) {
@@ -387,12 +387,18 @@ Plan plan(int batch, int co, int ci, long long n, int positions, int32_t dtype) 
     p.ct = ((ci + p.tiles_c - 1) / p.tiles_c + 15) / 16 * 16;
     p.steps = (long long)batch * ((n + positions - 1) / positions);
     const long long tiles = (long long)p.tiles_o * p.tiles_c;
-    p.slices = (int)std::max(1LL, std::min({ndc::num_sms() / tiles, (p.steps * positions + 511) / 512, 65535LL}));
+    long long slices = std::max(1LL, std::min(ndc::num_sms() / tiles, (p.steps * positions + 511) / 512));
     if (dtype == NDC_F32) {
         const long long most = (long long)kChain / (KP / 16) * leading_of(columns_of(p.ct));       // steps
-        p.slices = (int)std::max((long long)p.slices, std::min(65535LL, (p.steps + most - 1) / most));
+        slices = std::max(slices, (p.steps + most - 1) / most);
     }
+    p.passes = plan_passes(slices, (size_t)co * (ci + 1) * sizeof(float), tiles);
     return p;
+}
+
+bool too_large(int batch, int co, int ci, long long n) {
+    return n > 0x7fffffffLL - 2 * KP || (long long)batch * std::max(ci, co) > 0x7fffffffLL - MT || (n + KP - 1) / KP > 0x7fffffffLL / batch ||
+           ci > 65535 * (kMostColumns - 16) || (long long)co * (ci + 1LL) > (1LL << 35);
 }
 
 // Rows of n bfloat16 values, boxes of 128 rows of 64.
@@ -416,18 +422,18 @@ cudaError_t launch(const WgradArgs& A, const Plan& p, cudaStream_t st) {
     const int stages = stages_of<S>(p.ct);
     CUtensorMap map{};
     if (S::TMA && !make_gradient_map(map, A.gy, (long long)A.steps / A.steps_n * A.co, A.n)) return cudaErrorInvalidValue;
-    kern<<<dim3(p.tiles_o, p.tiles_c, p.slices), kThreads, 1024 + kHeader + (size_t)stages * S::bytes(columns_of(p.ct)), st>>>(map, A, stages);
+    kern<<<dim3(p.tiles_o, p.tiles_c, p.passes.each), kThreads, 1024 + kHeader + (size_t)stages * S::bytes(columns_of(p.ct)), st>>>(map, A, stages);
     ndc::launched();
     return cudaGetLastError();
 }
 
 template <typename T, typename TB>
-void launch_sum(const WgradArgs& A, void* gw, void* gb, cudaStream_t st) {
+void launch_sum(const WgradArgs& A, const float* partial, int slices, void* gw, void* gb, cudaStream_t st) {
     const long long n = (long long)A.co * A.width;
     // a chain of up to 16 loads per thread is no longer than the other kernel's, as soon as the elements fill the GPU
-    if (A.slices <= 16 && n >= 65536 && A.width <= 32 * 65535)
-        wgrad_few_kernel<T, TB><<<dim3((A.co + 31) / 32, (A.width + 31) / 32), 256, 0, st>>>(A.partial, A.slices, A.co, A.ci, A.width, (T*)gw, (TB*)gb);
-    else wgrad_sum_kernel<T, TB><<<(unsigned)((n + 31) / 32), 256, 0, st>>>(A.partial, A.slices, A.co, A.ci, A.width, (T*)gw, (TB*)gb);
+    if (slices <= 16 && n >= 65536 && A.width <= 32 * 65535)
+        wgrad_few_kernel<T, TB><<<dim3((A.co + 31) / 32, (A.width + 31) / 32), 256, 0, st>>>(partial, slices, A.co, A.ci, A.width, (T*)gw, (TB*)gb);
+    else wgrad_sum_kernel<T, TB><<<(unsigned)((n + 31) / 32), 256, 0, st>>>(partial, slices, A.co, A.ci, A.width, (T*)gw, (TB*)gb);
     ndc::launched();
 }
 
@@ -440,9 +446,9 @@ using namespace ndc::q8;
 extern "C" {
 
 size_t ndc_q8_wgrad_workspace_bytes(int32_t batch, int32_t co, int32_t ci, int64_t n, int32_t dtype) {
-    if (batch <= 0 || co <= 0 || ci <= 0 || n <= 0) return 0;
+    if (batch <= 0 || co <= 0 || ci <= 0 || n <= 0 || too_large(batch, co, ci, n)) return 0;
     // the most that either step asks for
-    return (size_t)std::max(plan(batch, co, ci, n, KP, dtype).slices, plan(batch, co, ci, n, 2 * KP, dtype).slices) * co * (ci + 1) * sizeof(float);
+    return std::max(plan(batch, co, ci, n, KP, dtype).passes.places(), plan(batch, co, ci, n, 2 * KP, dtype).passes.places()) * co * (ci + 1) * sizeof(float);
 }
 
 int ndc_q8_wgrad(int32_t batch, int32_t co, int32_t ci, int64_t n, int32_t dtype, const void* gy, const void* values, const void* scales,
@@ -456,24 +462,35 @@ int ndc_q8_wgrad(int32_t batch, int32_t co, int32_t ci, int64_t n, int32_t dtype
         return fail(NDC_ERR_ALIGNMENT, "q8 weight gradient: a tensor does not lie on its elements' size");
     const bool vec = vectors(n, dtype, gy);
     const int positions = positions_of(dtype, vec);
+    if (too_large(batch, co, ci, n)) return fail(NDC_ERR_UNSUPPORTED, "q8 weight gradient: problem too large");
     const Plan p = plan(batch, co, ci, n, positions, dtype);
-    if (n > 0x7fffffffLL - 2 * KP || (long long)batch * std::max(ci, co) > 0x7fffffffLL - MT || p.steps > 0x7fffffffLL || p.tiles_c > 65535 || (long long)co * (ci + 1) > (1LL << 35))
-        return fail(NDC_ERR_UNSUPPORTED, "q8 weight gradient: problem too large");
     const size_t need = ndc_q8_wgrad_workspace_bytes(batch, co, ci, n, dtype);
     if (!workspace || workspace_bytes < need) return fail(NDC_ERR_WORKSPACE, "q8 weight gradient: workspace of %zu bytes needed", need);
     if (ndc::tc::take_expired()) return fail(NDC_ERR_TIMEOUT, "a wait inside a kernel of an earlier call ran out after one second");
-    WgradArgs A{gy, (const unsigned char*)values, (const unsigned char*)scales, (float*)workspace, n, pitch_of(n), (int)scales_of(n), co, ci, p.ct,
-                ci + (gb ? 1 : 0), (int)((n + positions - 1) / positions), p.steps, p.slices, nullptr};
+    const int width = ci + (gb ? 1 : 0);
+    const size_t place = (size_t)co * width;
+    float* const places = (float*)workspace;
+    WgradArgs A{gy, (const unsigned char*)values, (const unsigned char*)scales, places + p.passes.first() * place, n, pitch_of(n), (int)scales_of(n), co, ci, p.ct,
+                width, (int)((n + positions - 1) / positions), p.steps, p.passes.slices, 0, nullptr};
     cudaError_t e = ndc::tc::expired_word(A.expired);
     if (e != cudaSuccess) return fail(NDC_ERR_CUDA, "q8 weight gradient: %s", cudaGetErrorString(e));
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == NDC_F32) e = vec ? launch<float, true>(A, p, st) : launch<float, false>(A, p, st);
-    else e = vec ? launch<bf16, true>(A, p, st) : launch<bf16, false>(A, p, st);
-    if (e == cudaSuccess) {
+    for (int i = 0; i < p.passes.count() && e == cudaSuccess; ++i) {
+        A.slice0 = i * p.passes.each;
+        if (dtype == NDC_F32) e = vec ? launch<float, true>(A, p, st) : launch<float, false>(A, p, st);
+        else e = vec ? launch<bf16, true>(A, p, st) : launch<bf16, false>(A, p, st);
+        if (e != cudaSuccess) break;
+        const float* from = places + p.passes.from(i) * place;
+        const int added = p.passes.added(i);
+        if (i + 1 < p.passes.count()) {
+            if (ndc_proj_sum(added, (int64_t)place, NDC_F32, from, places + p.passes.to(i) * place, stream) != NDC_OK)
+                return fail(NDC_ERR_CUDA, "q8 weight gradient: %s", ndc_proj_last_error());
+            continue;
+        }
         const bool wide = gb && gb_dtype == NDC_F32;
-        if (dtype == NDC_F32) { if (gb && !wide) launch_sum<float, bf16>(A, gw, gb, st); else launch_sum<float, float>(A, gw, gb, st); }
-        else if (wide) launch_sum<bf16, float>(A, gw, gb, st);
-        else launch_sum<bf16, bf16>(A, gw, gb, st);
+        if (dtype == NDC_F32) { if (gb && !wide) launch_sum<float, bf16>(A, from, added, gw, gb, st); else launch_sum<float, float>(A, from, added, gw, gb, st); }
+        else if (wide) launch_sum<bf16, float>(A, from, added, gw, gb, st);
+        else launch_sum<bf16, bf16>(A, from, added, gw, gb, st);
         e = cudaGetLastError();
     }
     return e == cudaSuccess ? NDC_OK : fail(NDC_ERR_CUDA, "q8 weight gradient: %s", cudaGetErrorString(e));

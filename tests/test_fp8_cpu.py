@@ -172,3 +172,18 @@ def test_the_forward_in_parts_refuses_bad_arguments(lib, status, call):
 def test_the_rounded_bias_refuses_bad_arguments(lib, status, call):
     assert call(lib) == status, lib.ndc_bias_last_error()
     assert lib.ndc_bias_last_error().startswith(b"bias")
+
+
+@pytest.mark.parametrize("batch,co,ci,n", [(2, 2048, 512, 64 ** 3), (1, 1024, 1024, 64 ** 3), (1, 256, 256, 1 << 22), (1, 8, 8, 1 << 28), (16, 2048, 2048, 8192), (4, 4096, 4096, 1 << 18)])
+def test_scratch_of_long_sums_is_bounded(lib, batch, co, ci, n):
+    """float32 sums in slices of some hundred positions each: three results of scratch or 64 MiB, whatever the positions."""
+    most = max(3 * 4 * co * (ci + 1), 64 << 20)
+    for dtype in (0, 1):
+        assert 0 < lib.ndc_q8_wgrad_workspace_bytes(batch, co, ci, n, dtype) <= most
+        assert 0 < lib.ndc_q8_product_workspace_bytes(batch, ci, co, n, dtype) <= most
+
+
+def test_scratch_of_what_is_refused(lib):
+    for size in ((1, 2 ** 31 - 1, 8, 64), (1, 8, 2 ** 31 - 1, 64), (2, 8, 8, 2 ** 31), (1, 2 ** 20, 2 ** 20, 64), (2 ** 20, 8, 8, 2 ** 20)):
+        assert lib.ndc_q8_wgrad_workspace_bytes(*size, 0) == 0
+        assert lib.ndc_q8_wgrad(*size, 0, A, A, A, A, None, 0, A, 1 << 40, None) == 2
