@@ -213,9 +213,9 @@ int columns_of(long long m, long long n, long long slices) {
 // counts 9 and 6, a launch to add slices up 6, and a slice's results are written and read.  At 2048 x 512 of 65536 (all slices
 // and their sum) 4 slices take 75 us, 5 106, 7 88 and 9 73; the model says 73, 108, 84 and 71.  2048 x 512 of 1024 takes 7 us in
 // one slice, 11 in two.  For float32 results a slice has 32 blocks at most: the MMA cuts its sums off, and a chain of 128 shrinks
-// by about 128 2^-25.
+// by 128 2^-25 to 128 2^-24; for bfloat16 ones 256, 2^-14.
 Passes plan_slices(int samples, long long m, long long n, long long k, int32_t dtype) {
-    const long long total = (long long)samples * ((k + KT - 1) / KT), least = dtype == NDC_F32 ? (total + 31) / 32 : 1, most = std::max(least, (total + 3) / 4);
+    const long long total = (long long)samples * ((k + KT - 1) / KT), chain = dtype == NDC_F32 ? 32 : 256, least = (total + chain - 1) / chain, most = std::max(least, (total + 3) / 4);
     long long best = least;
     double best_time = 1e300;
     auto consider = [&](long long slices) {

@@ -6,8 +6,9 @@
 // products are those of bfloat16 operands, exact in float32, and summed in float32 on the tensor cores.  float32
 // gradients go as three bfloat16 terms of eight bits each, which together are the value: three products instead of the six
 // of two split operands.  The MMA cuts its sums off towards zero, by up to 2^-24 of them each time, so that a chain of m shrinks by
-// about m 2^-25: float32 sums go into several accumulators in turn (as many as TMEM has room for), the small terms' into one of
-// their own, and a slice is no longer than kChain in each (2 x (11 -> 63) channels x 80000 positions: 1.5e-5 of the result in one chain).  The bias gradient comes from sixteen more columns of the product, of rows of ones.
+// m 2^-25 to m 2^-24 (values of one sign): sums go into several accumulators in turn (as many as TMEM has room for), float32's small terms' into one of
+// their own, and a slice is no longer than kChain or kChain16 in each (float32, 2 x (11 -> 63) channels x 80000 positions: 1.5e-5 of the result in
+// one chain; bfloat16, (256 -> 1000) x 2^20: 4.3e-4, where the rounding of the result is 2^-9 of it on the average).  The bias gradient comes from sixteen more columns of the product, of rows of ones.
 // 2 x (64 -> 256) x 64^3 in bfloat16: 62 us and 4 for the slices' sums (303 MB, 4.9 TB/s), bound by memory and by the held rows' way
 // through registers; 5 x (24 -> 96) of 203x171 in float32: 40 us, by loads of gy one value at a time and their split.
 //
@@ -38,6 +39,7 @@ constexpr int kRowBytes = 2 * KP;
 constexpr int kMostColumns = 256;             // of a tile, with the ones' 16
 constexpr int kTmem = 512;
 constexpr int kChain = 64;                    // MMAs of float32's leading terms into one accumulator
+constexpr int kChain16 = 1024;                // of bfloat16's: 2^-14 of a sum at most (2^-18 of a bias gradient's, of sixteen rows), rounded to 2^-8
 constexpr int kHeader = 1024;
 
 struct WgradArgs {
@@ -63,8 +65,11 @@ template <typename T, bool VEC> struct Step {
 };
 // columns of a tile's product
 __host__ __device__ inline int columns_of(int ct) { return ct + 16; }
-// Accumulators of float32's leading terms: what TMEM has room for beside that of the small ones, whole 32 columns read past their end.
-__host__ __device__ inline int leading_of(int columns) { return (kTmem - 16) / columns - 1 < 1 ? 1 : ((kTmem - 16) / columns - 1 > 15 ? 15 : (kTmem - 16) / columns - 1); }
+// Accumulators that sums go into in turn: what TMEM has room for (float32: beside that of the small terms), whole 32 columns read past their end.
+__host__ __device__ inline int leading_of(int columns, int terms) {
+    const int n = (kTmem - 16) / columns - (terms > 1 ? 1 : 0);
+    return n < 1 ? 1 : n > 15 ? 15 : n;
+}
 template <typename S> int stages_of(int ct) { return std::min(6, (int)((227 * 1024 - 1024 - kHeader) / S::bytes(columns_of(ct)))); }
 
 // Eight positions of a row of gy; zeros past its end.
@@ -234,8 +239,8 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
         tc_fence_after();
         const int quarter = warp & 3, o = o0 + 32 * quarter + lane;
         float* out = P.partial + (long long)blockIdx.z * P.width * P.co + o;
-        // float32: the small terms, then the leading ones of every step in turn
-        const int sums = S::TERMS > 1 ? 1 + min(steps, leading_of(columns)) : 1;
+        // float32's small terms, then the accumulators of every step in turn
+        const int sums = (S::TERMS > 1 ? 1 : 0) + min(steps, leading_of(columns, S::TERMS));
 #pragma unroll 1
         for (int k = 32 * (warp >> 2); k < columns; k += 8 * kStageWarps) {
             float v[32];
@@ -284,8 +289,8 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
     } else if (warp == kStageWarps) {
         if (elect()) {
             const unsigned idesc = instr_desc(columns);
-            const int leading = S::TERMS > 1 ? leading_of(columns) : 1;      // accumulators of the leading terms
-            int lead = columns;                                             // the next one's first column
+            const int leading = leading_of(columns, S::TERMS), lead0 = S::TERMS > 1 ? columns : 0;
+            int lead = lead0;                                               // first column of the step's accumulator
             for (int t = 0; t < steps; ++t) {
                 const int s = t % stages;
                 ok = mbar_wait_thread(full + 8 * s, (t / stages) & 1, kWaitLimit);
@@ -302,12 +307,12 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
 #pragma unroll
                             for (int i = 0; i < KP / 16; ++i) {
                             const bool small = S::TERMS > 1 && term > 0;
-                            const unsigned to = tmem + (S::TERMS > 1 && !small ? lead : 0);
+                            const unsigned to = tmem + (small ? 0 : lead);
                             const bool begun = small ? t > 0 || i > 0 || term < S::TERMS - 1 : t >= leading || sub > 0 || i > 0;
                             mma(to, g0 + (sub * S::G + term * MT * kRowBytes) / 16 + 2 * i, x + 2 * i, idesc, begun);
                         }
                     }
-                    lead = lead == leading * columns ? columns : lead + columns;
+                    lead = lead == lead0 + (leading - 1) * columns ? lead0 : lead + columns;
                     mma_commit(empty + 8 * s);
                 }
             }
@@ -388,9 +393,12 @@ Plan plan(int batch, int co, int ci, long long n, int positions, int32_t dtype) 
     p.steps = (long long)batch * ((n + positions - 1) / positions);
     const long long tiles = (long long)p.tiles_o * p.tiles_c;
     long long slices = std::max(1LL, std::min(ndc::num_sms() / tiles, (p.steps * positions + 511) / 512));
-    if (dtype == NDC_F32) {
-        const long long most = (long long)kChain / (KP / 16) * leading_of(columns_of(p.ct));       // steps
-        slices = std::max(slices, (p.steps + most - 1) / most);
+    const int chain = dtype == NDC_F32 ? kChain : kChain16, terms = dtype == NDC_F32 ? 3 : 1;
+    const long long most = (long long)chain / (positions / 16) * leading_of(columns_of(p.ct), terms);          // steps
+    if (slices * most < p.steps) {        // more slices than the GPU has room for at once: the ones that fit the same rounds of CTAs
+        slices = (p.steps + most - 1) / most;
+        const long long sms = ndc::num_sms(), rounds = (slices * tiles + sms - 1) / sms;
+        slices = std::max(slices, rounds * sms / tiles);      // (256 -> 1000) x 2^20 in bfloat16: 27 slices 1068 us, 22 1265, 9 1080
     }
     p.passes = plan_passes(slices, (size_t)co * (ci + 1) * sizeof(float), tiles);
     return p;
