@@ -728,7 +728,7 @@ void held_product(int64_t samples, int64_t m, int64_t n, int64_t k, const Held& 
 // launch first, under which the host gets ahead.)
 template <class F>
 void held_project(const Tensor& x, int64_t batch, int64_t ci, int64_t co, int64_t n, F hold_w, const Tensor& bias, Tensor& y, Held* rows = nullptr) {
-    if (ci > 512 || n > (1 << 24)) {
+    if (ci > 512) {
         const Held h = hold_channels(x, batch, ci, n, rows);
         return held_product(1, batch * n, co, ci, h, hold_w(), bias, n, y, false);
     }
@@ -893,6 +893,7 @@ struct HeldLinearNode : public torch::autograd::Function<HeldLinearNode> {
 
 Tensor linear_q8(const Tensor& x_in, const Tensor& w_in, const std::optional<Tensor>& bias_in, bool products) {
     check_linear(x_in, w_in, bias_in);
+    TORCH_CHECK(!products || slabs(x_in).n <= 1 << 24, "deconver_b200: products in 8 bits take inputs of up to 2^24 positions per sample, not ", x_in.sizes());
     c10::cuda::CUDAGuard guard(x_in.device());
     const Tensor x = x_in.contiguous(), w = w_in.contiguous(), b = bias_in ? *bias_in : Tensor();
     refuse_tangents({&x, &w, &b});

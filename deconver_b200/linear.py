@@ -49,7 +49,7 @@ def channel_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     products="fp8": the products are of operands held in 8 bits, in blocks of 128 along what they are summed over:
         y (blocks of input channels), the input's gradient (of output channels), the weight's (of positions, from the
         checkpoint, so that the input is kept in 8 bits here too).  Sums are float32; the bias and its gradient are not
-        held in 8 bits.
+        held in 8 bits.  Up to 2^24 positions per sample.
     """
     eight = is_fp8(checkpoint, "checkpoint"), is_fp8(products, "products")
     operands = native_operands(x, weight)

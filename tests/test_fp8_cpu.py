@@ -187,3 +187,12 @@ def test_scratch_of_what_is_refused(lib):
     for size in ((1, 2 ** 31 - 1, 8, 64), (1, 8, 2 ** 31 - 1, 64), (2, 8, 8, 2 ** 31), (1, 2 ** 20, 2 ** 20, 64), (2 ** 20, 8, 8, 2 ** 20)):
         assert lib.ndc_q8_wgrad_workspace_bytes(*size, 0) == 0
         assert lib.ndc_q8_wgrad(*size, 0, A, A, A, A, None, 0, A, 1 << 40, None) == 2
+
+
+def test_products_of_too_many_positions_are_refused(lib):
+    """By the layer, before a kernel's own limit is met."""
+    x, w = torch.zeros(1, 1, 1).expand(1, 1, 2 ** 24 + 1), torch.zeros(4, 1, 1)
+    with pytest.raises(RuntimeError, match="up to 2.24 positions per sample"):
+        _lib.load_ext().linear_q8(x, w, None, True)
+    with pytest.raises(RuntimeError, match="up to 2.24 positions per sample"):
+        _lib.load_ext().linear_q8(x.view(1, 1, -1, 1), w, None, True)
