@@ -56,7 +56,12 @@ def channel_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     if not any(eight):
         if operands is not None and (bias is not None or operands[0].dtype == torch.bfloat16):
             return native("linear", (*operands, bias))
-        return F.conv1d(x.flatten(2), weight, bias).view(x.shape[0], -1, *x.shape[2:])
+        if x.numel() and weight.numel():
+            y = F.conv1d(x.flatten(2), weight, bias)
+        else:                                   # a convolution refuses it, or gives no outputs
+            y = weight[:, :, 0] @ x.flatten(2)
+            y = y if bias is None else y + bias[:, None]
+        return y.view(x.shape[0], weight.shape[0], *x.shape[2:])
     if operands is None:
         raise RuntimeError("deconver_b200: linear in 8 bits takes CUDA float32 / bfloat16 tensors (batch, channels, spatial...) and a weight of "
                            f"their type, not {x.dtype} {tuple(x.shape)} on {x.device} and {weight.dtype} on {weight.device}")

@@ -196,3 +196,14 @@ def test_products_of_too_many_positions_are_refused(lib):
         _lib.load_ext().linear_q8(x, w, None, True)
     with pytest.raises(RuntimeError, match="up to 2.24 positions per sample"):
         _lib.load_ext().linear_q8(x.view(1, 1, -1, 1), w, None, True)
+
+
+@pytest.mark.parametrize("with_bias", [True, False])
+@pytest.mark.parametrize("shape,outputs", [((0, 4, 5), 8), ((2, 4, 0), 8), ((2, 0, 5), 8), ((2, 4, 3, 0, 2), 8), ((2, 4, 5), 0), ((0, 4, 0, 3), 0)], ids=str)
+def test_the_exact_layer_of_no_elements(shape, outputs, with_bias):
+    x, w, b = (torch.ones(s, requires_grad=True) for s in (shape, (outputs, shape[1], 1), (outputs,)))
+    y = dcb.channel_linear(x, w, b if with_bias else None)
+    assert y.shape == (shape[0], outputs, *shape[2:]) and (y == float(with_bias)).all()
+    y.sum().backward()
+    assert not x.grad.any() and not w.grad.any()
+    assert not with_bias or torch.equal(b.grad, torch.full((outputs,), float(y[:, :1].numel())))
