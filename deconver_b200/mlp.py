@@ -11,9 +11,11 @@ reduction: two extra trips over the hidden tensor.  CPU tensors and other dtypes
 sequence.
 
 ``checkpoint="fp8"`` keeps what the backward pass needs (the inputs of both projections and the hidden tensor before the
-GELU) in 8 bits, ``products="fp8"`` computes the projections from operands held in 8 bits: see `channel_linear`.
+GELU) in 8 bits, ``products="fp8"`` computes the projections from operands held in 8 bits: see `channel_linear`.  A block whose
+first two modules were replaced by others than a `Linear` and an erf-form GELU keeps its hidden tensor as they do, with a warning.
 """
 
+import warnings
 from typing import Optional
 
 import torch
@@ -61,6 +63,9 @@ class MLP(nn.Module):
         first, act, drop1, second, drop2 = self.block
         operands = native_operands(x, first.linear.weight) if type(first) is Linear else None
         if operands is None or not isinstance(act, nn.GELU) or act.approximate != "none":
+            if self.checkpoint == "fp8" and (operands is not None or type(first) is not Linear):
+                warnings.warn("deconver_b200: MLP(checkpoint='fp8') keeps the hidden tensor exactly: its block does not begin with a Linear and an "
+                              "erf-form GELU", RuntimeWarning, stacklevel=2)
             return self.block(x)
         if first.eight:
             h = channel_linear(x, first.linear.weight, checkpoint=first.checkpoint, products=first.products)

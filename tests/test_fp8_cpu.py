@@ -207,3 +207,20 @@ def test_the_exact_layer_of_no_elements(shape, outputs, with_bias):
     y.sum().backward()
     assert not x.grad.any() and not w.grad.any()
     assert not with_bias or torch.equal(b.grad, torch.full((outputs,), float(y[:, :1].numel())))
+
+
+def test_an_mlp_that_keeps_its_hidden_tensor_says_so():
+    import warnings
+
+    class Same(torch.nn.Module):
+        def forward(self, x):
+            return x
+
+    x = torch.randn(1, 4, 3)
+    for checkpoint in ("exact", "fp8"):
+        mlp = dcb.MLP(4, checkpoint=checkpoint)
+        mlp.block[0], mlp.block[3] = Same(), Same()
+        with warnings.catch_warnings(record=True) as told:
+            warnings.simplefilter("always")
+            assert torch.equal(mlp(x), torch.nn.functional.gelu(x))
+        assert [str(w.message).count("keeps the hidden tensor exactly") for w in told] == [1] * (checkpoint == "fp8")
