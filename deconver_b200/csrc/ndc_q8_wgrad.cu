@@ -129,7 +129,7 @@ __device__ __forceinline__ unsigned decode_bf16(unsigned pair, float scale) {
     return *reinterpret_cast<const unsigned*>(&p);
 }
 
-// The sum of a row of gy over some steps, by a warp.
+// The sum of a row of gy over some steps, by a warp; no further than to what makes it NaN.
 template <typename T>
 __device__ __forceinline__ float row_sum(const WgradArgs& P, int o, long long first, int steps, int positions, int lane) {
     float s = 0.0f;
@@ -137,6 +137,8 @@ __device__ __forceinline__ float row_sum(const WgradArgs& P, int o, long long fi
         const long long sample = step / P.steps_n, p = (step - sample * P.steps_n) * positions, left = min((long long)positions, P.n - p);
         const T* g = reinterpret_cast<const T*>(P.gy) + (sample * P.co + o) * P.n + p;
         for (int i = lane; i < left; i += 32) s += ndc::to_f32(g[i]);
+        const float inf = __uint_as_float(kInfinite);
+        if (__any_sync(0xffffffffu, s != s) || (__any_sync(0xffffffffu, s == inf) && __any_sync(0xffffffffu, s == -inf))) return __uint_as_float(0x7fffffffu);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
