@@ -64,6 +64,8 @@ __device__ __forceinline__ unsigned long long positions_desc(unsigned addr) {
            2ull << 61;
 }
 
+// PARTS: of the outputs, in the grid's y.  (One part by the same code took 2 - 4 % more: 167 us for 161 at 2 x (256 -> 64) x 64^3.)
+template <bool PARTS>
 __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                               const __grid_constant__ CUtensorMap map_y, const __grid_constant__ ForwardArgs P) {
     extern __shared__ unsigned char raw_smem[];
@@ -73,7 +75,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
     const int weights = P.blocks * P.columns * 128;                       // bytes
     const unsigned w_at = base + kHeader, y_at = w_at + weights, x_at = y_at + 2 * P.staged * kStaged;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int o0 = blockIdx.y * P.columns;                                // the part's first output
+    const int o0 = PARTS ? blockIdx.y * P.columns : 0;                    // the part's first output
     if (threadIdx.x == 0) {
         for (int i = 0; i < P.slots; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1 + (P.values ? kHoldWarps : 0)); }
         for (int i = 0; i < 2; ++i) { mbar_init(dfull + 8 * i, 1); mbar_init(dempty + 8 * i, kStoreWarps); }
@@ -82,7 +84,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
     }
     if (threadIdx.x < 2) reinterpret_cast<volatile unsigned*>(smem + kGaveUp)[threadIdx.x] = 0u;
     if (warp == 0) tmem_alloc(slot_at, 512);
-    for (int j = threadIdx.x; j < (kHeader - kBias) / 4; j += kThreads) reinterpret_cast<float*>(smem + kBias)[j] = P.bias && j < P.columns && o0 + j < P.co ? load_bias(P.bias, P.bias_bf16, o0 + j) : 0.0f;
+    for (int j = threadIdx.x; j < (kHeader - kBias) / 4; j += kThreads) reinterpret_cast<float*>(smem + kBias)[j] = P.bias && (!PARTS || j < P.columns) && o0 + j < P.co ? load_bias(P.bias, P.bias_bf16, o0 + j) : 0.0f;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
                 fence_async_proxy();
                 group_sync(group);
                 const int o = o0 + u / 2 * MT;
-                if (copies) tma_store3(&map_y, p + (u & 1) * 64, o, sample, y_at + (group * P.staged + place) * kStaged, p + (u & 1) * 64 < P.n && o < P.co);
+                if (copies) tma_store3(&map_y, p + (u & 1) * 64, o, sample, y_at + (group * P.staged + place) * kStaged, p + (u & 1) * 64 < P.n && (!PARTS || o < P.co));
                 if (++place == P.staged) place = 0;
             }
         }
@@ -144,16 +146,18 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
         for (int t = blockIdx.x; P.values && t < P.tiles && ok; t += gridDim.x) {
             const int sample = t / P.tiles_n, k = t - sample * P.tiles_n;
             const long long p = (long long)k * kBlock + 8 * l;
-            unsigned turn = (unsigned)t % gridDim.y * P.blocks % gridDim.y;        // the part that has the tile's first block
+            [[maybe_unused]] unsigned turn = PARTS ? (unsigned)t % gridDim.y * P.blocks % gridDim.y : 0;      // the part that has the tile's first block
             for (int block = 0; block < P.blocks; ++block) {
                 ok = mbar_wait(full + 8 * slot, phase);
                 if (!ok) break;
-                const bool mine = turn == blockIdx.y;
-                if (++turn == gridDim.y) turn = 0;
-                if (!mine) {
-                    if (lane == 0) mbar_arrive(empty + 8 * slot);
-                    if (++slot == P.slots) { slot = 0; phase ^= 1; }
-                    continue;
+                if constexpr (PARTS) {
+                    const bool mine = turn == blockIdx.y;
+                    if (++turn == gridDim.y) turn = 0;
+                    if (!mine) {
+                        if (lane == 0) mbar_arrive(empty + 8 * slot);
+                        if (++slot == P.slots) { slot = 0; phase ^= 1; }
+                        continue;
+                    }
                 }
                 const unsigned char* from = smem + (x_at - base) + slot * kBlockBytes + (l >> 3) * kHalf;
                 uint4 q[KC / (2 * kHoldWarps)];
@@ -316,9 +320,10 @@ int launch_forward(int batch, int ci, int co, long long n, Parts parts, const vo
     if (e != cudaSuccess) return fail(NDC_ERR_CUDA, "q8 linear: %s", cudaGetErrorString(e));
     CUtensorMap map_x, map_w, map_y;
     if (!make_tensor_map(map_x, x, 2, batch, ci, n, KC) || !make_tensor_map(map_y, y, 2, batch, co, n, MT) || !make_weight_map(map_w, w, co, ci)) return fail(NDC_ERR_CUDA, "q8 linear: the driver refused a tensor map");
-    e = ndc::allow_smem(forward_kernel);
+    const auto kern = parts.parts > 1 ? forward_kernel<true> : forward_kernel<false>;
+    e = ndc::allow_smem(kern);
     if (e == cudaSuccess) {
-        forward_kernel<<<dim3(ctas_of(P.tiles, parts.parts), parts.parts), kThreads,
+        kern<<<dim3(ctas_of(P.tiles, parts.parts), parts.parts), kThreads,
                          1024 + kHeader + weights + (size_t)2 * P.staged * kStaged + (size_t)P.slots * kBlockBytes, (cudaStream_t)stream>>>(map_x, map_w, map_y, P);
         ndc::launched();
         e = cudaGetLastError();
