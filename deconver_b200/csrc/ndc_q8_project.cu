@@ -369,8 +369,7 @@ int ndc_q8_project(int32_t batch, int32_t ci, int32_t co, int64_t n, int32_t dty
     const int parts = plan_parts(tiles, (co + MT - 1) / MT, blocks);
     ProjectArgs P{x, (const unsigned char*)w_scales, bias, bias_dtype == NDC_BF16, y, n, ci, co, blocks, (co + MT - 1) / MT, (int)tiles_n, parts, (int)(tiles * parts),
                   0, 0, Divider((unsigned)tiles_n), Divider((unsigned)parts), Divider((unsigned)blocks), nullptr};
-    // A w of up to four blocks stays.  One that goes around needs many on their way, and the tile's blocks change seldom.  Loads
-    // in flight need room in the L1 cache, which is what shared memory leaves
+    // A w of up to four blocks stays.  One that goes around needs many on their way, and the tile's blocks change seldom.
     P.resident = P.parts == 1 && P.chunks * blocks <= kMostBlocks;
     P.stages = P.resident ? P.chunks * blocks : kOperands - kSlots;
     cudaError_t e = ndc::tc::expired_word(P.expired);

@@ -5,10 +5,12 @@
 // for what is held, v.  Every held value is a bfloat16 value (four significant bits and a power of two), so the
 // products are those of bfloat16 operands, exact in float32, and summed in float32 on the tensor cores.  float32
 // gradients go as three bfloat16 terms of eight bits each, which together are the value: three products instead of the six
-// of two split operands.  The MMA cuts its sums off towards zero, by up to 2^-24 of them each time, so that a chain of m shrinks by
+// of two split operands.  The MMA cuts its sums off towards zero, by up to 2^-23 of them each time, so that a chain of m shrinks by
 // m 2^-25 to m 2^-24 (values of one sign): sums go into several accumulators in turn (as many as TMEM has room for), float32's small terms' into one of
 // their own, and a slice is no longer than kChain or kChain16 in each (float32, 2 x (11 -> 63) channels x 80000 positions: 1.5e-5 of the result in
-// one chain; bfloat16, (256 -> 1000) x 2^20: 4.3e-4, where the rounding of the result is 2^-9 of it on the average).  The bias gradient comes from sixteen more columns of the product, of rows of ones.
+// one chain; bfloat16, (256 -> 1000) x 2^20: 4.3e-4, where the rounding of the result is 2^-9 of it on the average).  Slices whose sums would
+// be too much memory go in several launches (plan_passes).  The bias gradient comes from sixteen more columns of the product, of rows of ones; one
+// that is not finite is added up by itself.
 // 2 x (64 -> 256) x 64^3 in bfloat16: 62 us and 4 for the slices' sums (303 MB, 4.9 TB/s), bound by memory and by the held rows' way
 // through registers; 5 x (24 -> 96) of 203x171 in float32: 40 us, by loads of gy one value at a time and their split.
 //
