@@ -236,6 +236,11 @@ Passes plan_slices(int samples, long long m, long long n, long long k, int32_t d
     return plan_passes(best, (size_t)(m * n) * sizeof(float), ((m + MT - 1) / MT) * ((n + nt - 1) / nt));
 }
 
+bool too_large(int samples, long long m, long long n, long long k) {
+    return m > (0x7fffffffLL - 4 * MT) / samples || n > (0x7fffffffLL - 4 * MT) / samples || k > 0x7fffffffLL - KT || (k + KT - 1) / KT > 0x7fffffffLL / samples ||
+           (m + MT - 1) / MT > 0x7fffffffLL / ((n + 63) / 64);
+}
+
 }  // namespace
 }  // namespace q8
 }  // namespace ndc
@@ -245,7 +250,7 @@ using namespace ndc::q8;
 extern "C" {
 
 size_t ndc_q8_product_workspace_bytes(int32_t samples, int64_t m, int64_t n, int64_t k, int32_t dtype) {
-    if (samples <= 0 || m <= 0 || n <= 0 || k <= 0) return 0;
+    if (samples <= 0 || m <= 0 || n <= 0 || k <= 0 || too_large(samples, m, n, k)) return 0;
     return plan_slices(samples, m, n, k, dtype).places() * m * n * sizeof(float);
 }
 
@@ -255,10 +260,7 @@ int ndc_q8_product(int32_t samples, int64_t m, int64_t n, int64_t k, int32_t dty
     if (!a_values || !a_scales || !b_values || !b_scales || !out) return fail(NDC_ERR_INVALID, "q8 product: operands and out must not be NULL");
     if (samples <= 0 || m <= 0 || n <= 0 || k <= 0 || rows <= 0 || m % rows) return fail(NDC_ERR_INVALID, "q8 product: extents must be positive, m a multiple of rows");
     if ((dtype != NDC_F32 && dtype != NDC_BF16) || (bias && bias_dtype != NDC_F32 && bias_dtype != NDC_BF16)) return fail(NDC_ERR_INVALID, "q8 product: dtype must be NDC_F32 or NDC_BF16");
-    const long long kblocks = (k + KT - 1) / KT;
-    if (m > (0x7fffffffLL - 4 * MT) / samples || n > (0x7fffffffLL - 4 * MT) / samples || k > 0x7fffffffLL - KT || kblocks > 0x7fffffffLL / samples ||
-        (m + MT - 1) / MT > 0x7fffffffLL / ((n + 63) / 64))
-        return fail(NDC_ERR_UNSUPPORTED, "q8 product: problem too large");
+    if (too_large(samples, m, n, k)) return fail(NDC_ERR_UNSUPPORTED, "q8 product: problem too large");
     for (const void* p : {a_values, b_values})
         if ((uintptr_t)p & 15) return fail(NDC_ERR_ALIGNMENT, "q8 product: values must lie on 16 bytes");
     for (const void* p : {a_scales, b_scales})
@@ -277,7 +279,7 @@ int ndc_q8_product(int32_t samples, int64_t m, int64_t n, int64_t k, int32_t dty
     P.pitch_a = P.pitch_b = (int)scales_of(k);
     P.rows_a = (long long)samples * m; P.rows_b = (long long)samples * n;
     P.m = (int)m; P.n = (int)n; P.k = (int)k;
-    P.samples = samples; P.kblocks = (int)kblocks; P.slices = slices;
+    P.samples = samples; P.kblocks = (int)((k + KT - 1) / KT); P.slices = slices;
     P.bias = bias; P.bias_bf16 = bias_dtype == NDC_BF16; P.out = slices > 1 ? (float*)workspace + passes.first() * m * n : out; P.rows = rows;
     cudaError_t e = ndc::tc::expired_word(P.expired);
     if (e != cudaSuccess) return fail(NDC_ERR_CUDA, "q8 product: %s", cudaGetErrorString(e));

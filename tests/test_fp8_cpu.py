@@ -187,6 +187,9 @@ def test_scratch_of_what_is_refused(lib):
     for size in ((1, 2 ** 31 - 1, 8, 64), (1, 8, 2 ** 31 - 1, 64), (2, 8, 8, 2 ** 31), (1, 2 ** 20, 2 ** 20, 64), (2 ** 20, 8, 8, 2 ** 20)):
         assert lib.ndc_q8_wgrad_workspace_bytes(*size, 0) == 0
         assert lib.ndc_q8_wgrad(*size, 0, A, A, A, A, None, 0, A, 1 << 40, None) == 2
+    for samples, m, n, k in ((1, 2 ** 31, 2 ** 31, 8), (1, 2 ** 62, 4, 8), (2, 2 ** 30, 8, 8), (1, 2 ** 30, 2 ** 23, 8), (1, 8, 8, 2 ** 31), (2 ** 20, 8, 8, 2 ** 20)):
+        assert lib.ndc_q8_product_workspace_bytes(samples, m, n, k, 0) == 0
+        assert lib.ndc_q8_product(samples, m, n, k, 0, A, A, A, A, None, 0, m, A, A, 1 << 40, None) == 2
 
 
 def test_products_of_too_many_positions_are_refused(lib):
